@@ -323,7 +323,7 @@ int32_t crx_adamw_step(int32_t n, void *const *weights, float *const *masters, f
         k.beta2 = (float)a->beta2;
         k.one_less_beta1 = (float)(1.0 - a->beta1);
         k.one_less_beta2 = (float)(1.0 - a->beta2);
-        k.keep = (float)(1.0 - a->lr * a->weight_decay);
+        k.keep = 1.0 - a->lr * a->weight_decay;
         k.rate = (float)(a->lr / (1.0 - std::pow(a->beta1, (double)a->step)));
         k.root = (float)(1.0 / std::sqrt(1.0 - std::pow(a->beta2, (double)a->step)));
         k.eps = (float)a->eps;

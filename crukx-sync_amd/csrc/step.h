@@ -129,8 +129,8 @@ struct AdamList {
 };
 
 struct AdamArgs {
+    double keep;      // 1 - lr * weight_decay
     float beta1, beta2, one_less_beta1, one_less_beta2;
-    float keep;       // 1 - lr * weight_decay
     float rate;       // lr / (1 - beta1^step)
     float root;       // 1 / sqrt(1 - beta2^step)
     float eps;

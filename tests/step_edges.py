@@ -1,0 +1,57 @@
+"""Checks of the training step's operators that run on any device: on the GPU in tests/test_step_edges.py, and on the CPU
+model of the library in tests/model/run_step_edges.py.  Each takes the device's name."""
+
+from __future__ import annotations
+
+import torch
+
+import crukx_sync
+import step_reference as ref
+
+EDGES = {}
+
+
+def edge(check):
+    EDGES[check.__name__] = check
+    return check
+
+
+def _generator(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------ AdamW
+
+@edge
+def small_decays_shrink_the_masters(dev):
+    """lr * weight_decay far below the spacing of 32-bit numbers at 1, as at lr = 1e-6: a single master hardly shows it,
+    the projection of all changes on the masters does.
+
+    Every master is rounded once, by at most u |w|, in directions that do not depend on one another (the updates are random
+    and many times a last place); so the projection sum(w dw) / sum(w^2) is off by more than 8 u sqrt(sum w^4) / sum(w^2)
+    with a probability below 1e-13.  The decay itself is held to 1e-6 of itself beside that."""
+    n = 120_000 if dev == "cpu" else 4_000_000
+    g = _generator(1)
+    w0 = torch.randn(n, generator=g) * 0.02
+    m0, g0 = torch.randn(n, generator=g) * 1e-3, torch.randn(n, generator=g) * 1e-2
+    v0 = torch.rand(n, generator=g) * 1e-5
+    for wd in (0.01, 0.1, 0.0):
+        s = [{"p": t.clone().to(dev)} for t in (w0.bfloat16(), w0, m0, v0, g0)]
+        crukx_sync.adamw_step(*s, step=7, lr=1e-6, weight_decay=wd)
+        want = ref.adamw(w0, m0, v0, g0, 7, 1e-6, (0.9, 0.999), 1e-8, wd)[0]
+        got, w = s[1]["p"].cpu().double(), w0.double()
+        off = float(((got - want) * w).sum() / (w * w).sum())
+        allowed = 8 * ref.U * float((w ** 4).sum().sqrt() / (w * w).sum()) + 1e-6 * 1e-6 * wd
+        assert abs(off) <= allowed, f"decay {wd}: {off / (1e-6 * wd or 1):+.3f} of it too little (allowed {allowed / (1e-6 * wd or 1):.3f})"
+
+
+@edge
+def infinite_masters_stay_infinite(dev):
+    """As in the formula, with and without a decay; the neighbours are stepped as ever."""
+    w0 = torch.tensor([1.0, float("inf"), -2.0, float("-inf"), 0.0, 3e38])
+    for wd in (0.0, 0.1):
+        s = [{"p": t.clone().to(dev)} for t in (w0.bfloat16(), w0, torch.ones(6), torch.ones(6), torch.ones(6))]
+        crukx_sync.adamw_step(*s, step=3, lr=1e-3, weight_decay=wd)
+        one = torch.ones(6)
+        want = ref.adamw(w0, one, one, one, 3, 1e-3, (0.9, 0.999), 1e-8, wd)[0]
+        ref.same(s[1]["p"], want, 4 * ref.U * torch.where(w0.isfinite(), w0.abs() + 1e-2, 0.0))
