@@ -11,8 +11,9 @@ The reference leaves this step to its caller (its training loop, bench/grpo.py:5
 
 - All tensors lie on one HIP device.  Work is enqueued on the current stream; nothing waits for the device
   or reads from it, so the calls can be captured into a graph.
-- Wrong arguments raise ValueError before anything is enqueued.  What depends on values on the device cannot:
-  a token id outside the vocabulary makes its position's results and gradient NaN (and with them the loss).
+- Wrong arguments raise ValueError before anything is enqueued, and so do dual tensors (there are no
+  forward-mode derivatives).  What depends on values on the device cannot: a token id outside
+  the vocabulary makes its position's results and gradient NaN (and with them the loss).
 - A position whose mask is 0 takes no part: its logits and token id are not read (they may hold anything),
   its results are 0 and its gradient is 0.
 - Logits that are -inf, or the type's lowest value beside larger ones, have probability 0.  A row without a

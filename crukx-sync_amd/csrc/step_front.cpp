@@ -8,6 +8,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -46,8 +47,12 @@ bool g_any_device = false;       // the CPU model of the library: tensors in hos
 
 int64_t index_of(const Tensor &t) { return g_any_device ? 0 : t.is_cuda() ? (int64_t)t.device().index() : -1; }
 
+// A dual tensor's tangent would be lost without a word: no operator here has a forward-mode derivative.
+constexpr const char *kNoTangent = "forward-mode derivatives are not supported, got a dual tensor";
+
 void check_hip(const char *name, const Tensor &t) {
     if (!t.defined()) bad(std::string(name) + ": expected a torch tensor");
+    if (t._fw_grad(0).defined()) bad(std::string(name) + ": " + kNoTangent);
     if (index_of(t) < 0) bad(std::string(name) + ": expected a tensor on a HIP device, got one on " + t.device().str());
 }
 
@@ -280,6 +285,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const Tensor &x = kept[0];
         Tensor grad;
         if (up[0].defined()) {
+            check_hip("gradient", up[0]);
             const crx_logits in = logits_of(x, kept[1], kept[2], ctx->saved_data["temperature"].toDouble());
             const auto made = ctx->saved_data.find("grad");
             const bool first = made != ctx->saved_data.end();
@@ -353,6 +359,7 @@ struct List {
     std::vector<uint64_t> numel;
     std::vector<int32_t> type;
     Tensor one;  // the first of them
+    const bool duals = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // whether any tensor can be one
 
     explicit List(size_t n) {
         if (n > (size_t)INT32_MAX) bad("too many tensors");
@@ -374,6 +381,7 @@ struct List {
         } else if (impl->device() != one.device()) {
             fail("all tensors must be on one HIP device, got one on " + v.device().str());
         }
+        if (duals && v._fw_grad(0).defined()) fail(kNoTangent);
         if (impl->layout() != at::kStrided || !impl->is_contiguous()) fail("tensor must be contiguous");
         const int32_t k = type_of(v);
         if (k < 0 || (floats_only && k != CRX_F32)) fail(std::string("unexpected type ") + c10::toString(v.scalar_type()));

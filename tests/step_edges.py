@@ -3,6 +3,7 @@ model of the library in tests/model/run_step_edges.py.  Each takes the device's 
 
 from __future__ import annotations
 
+import pytest
 import torch
 
 import crukx_sync
@@ -55,3 +56,61 @@ def infinite_masters_stay_infinite(dev):
         one = torch.ones(6)
         want = ref.adamw(w0, one, one, one, 3, 1e-3, (0.9, 0.999), 1e-8, wd)[0]
         ref.same(s[1]["p"], want, 4 * ref.U * torch.where(w0.isfinite(), w0.abs() + 1e-2, 0.0))
+
+
+# ------------------------------------------------------------------ tensors that are more than their data
+
+def _positions(dev, shape=(3,), vocab=9, seed=2):
+    g = _generator(seed)
+    x = torch.randn((*shape, vocab), generator=g).to(dev)
+    y = torch.randint(0, vocab, shape, generator=g).to(dev)
+    f = torch.zeros(shape, device=dev)
+    return x, y, f
+
+
+def _calls(x, y, f):
+    """Every entry point by what it takes of a tensor: name -> (call of a tensor put in that place, the place's tensor)."""
+    state = lambda: [{"p": t.clone()} for t in (f, f, f, f, f)]  # noqa: E731
+
+    def adamw(k, t):
+        s = state()
+        s[k]["p"] = t
+        crukx_sync.adamw_step(*s, step=1, lr=1e-3)
+
+    return {
+        "scores": (lambda t: crukx_sync.token_logprobs(t, y), x),
+        "entropies": (lambda t: crukx_sync.token_logprobs(t, y, entropy=True), x),
+        "loss": (lambda t: crukx_sync.policy_loss(t, y, f, f), x),
+        "loss and gradient": (lambda t: crukx_sync.policy_loss_grad(t, y, f, f), x),
+        "old": (lambda t: crukx_sync.policy_loss(x, y, t, f), f),
+        "advantages": (lambda t: crukx_sync.policy_loss(x, y, f, t), f),
+        "ref": (lambda t: crukx_sync.policy_loss_grad(x, y, f, f, None, t), f),
+        "norm": (lambda t: crukx_sync.grad_norm([f, t]), f),
+        "norm of a mapping": (lambda t: crukx_sync.grad_norm({"a": t}), f),
+        "clip": (lambda t: crukx_sync.clip_grad_norm([t, f], 1.0), f),
+        "adamw weights": (lambda t: adamw(0, t), f), "adamw masters": (lambda t: adamw(1, t), f),
+        "adamw exp_avg": (lambda t: adamw(2, t), f), "adamw exp_avg_sq": (lambda t: adamw(3, t), f),
+        "adamw grads": (lambda t: adamw(4, t), f),
+    }
+
+
+@edge
+def forward_mode_derivatives_are_refused(dev):
+    """No operator has a forward-mode derivative: a dual tensor in any place raises, with and without requires_grad, and
+    does not come back as a result without a tangent."""
+    import torch.autograd.forward_ad as fwd
+    x, y, f = _positions(dev)
+    for name, (call, at) in _calls(x, y, f).items():
+        call(at.clone())
+        with fwd.dual_level():
+            for leaf in (False, True):
+                dual = fwd.make_dual(at.clone().requires_grad_(leaf and not name.startswith(("clip", "adamw"))), torch.ones_like(at))
+                with pytest.raises((ValueError, RuntimeError), match="forward-mode|jvp"):
+                    call(dual)
+            call(at.clone())  # a level by itself changes nothing
+    leaf = x.clone().requires_grad_()
+    with fwd.dual_level():
+        up = fwd.make_dual(f + 1, torch.ones_like(f))
+        for r, u in ((crukx_sync.token_logprobs(leaf, y), up), (crukx_sync.policy_loss(leaf, y, f, f).loss, up[0])):
+            with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
+                torch.autograd.grad(r, leaf, u)
