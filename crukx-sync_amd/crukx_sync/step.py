@@ -10,7 +10,8 @@
 The reference leaves this step to its caller (its training loop, bench/grpo.py:57-100, is plain torch).
 
 - All tensors lie on one HIP device.  Work is enqueued on the current stream; nothing waits for the device
-  or reads from it, so the calls can be captured into a graph.
+  or reads from it, so the calls can be captured into a HIP graph.  Tracers (torch.jit.trace, make_fx) do not see
+  kernels: under one the calls raise RuntimeError; torch.compile runs them between its graphs.
 - Wrong arguments raise ValueError before anything is enqueued, and so do dual tensors (there are no
   forward-mode derivatives).  What depends on values on the device cannot: a token id outside
   the vocabulary makes its position's results and gradient NaN (and with them the loss).

@@ -8,9 +8,11 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cstdint>
 #include <stdexcept>
@@ -46,6 +48,17 @@ bool g_any_device = false;       // the CPU model of the library: tensors in hos
 // -------------------------------------------------------------------- devices and calls
 
 int64_t index_of(const Tensor &t) { return g_any_device ? 0 : t.is_cuda() ? (int64_t)t.device().index() : -1; }
+
+// Under a tracer the calls must not run: it sees the allocation of their results and not the kernels, and what it records
+// would return memory that nothing has written.  (Modes that only look on, as profilers do, are not meant.)
+void not_traced() {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    bool traced = torch::jit::tracer::isTracing();
+    for (auto mode : {TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FAKE, TorchDispatchModeKey::FUNCTIONAL})
+        traced = traced || TorchDispatchModeTLS::get_mode(mode).has_value();
+    if (traced) throw std::runtime_error("the training step's calls cannot be traced");
+}
 
 // A dual tensor's tangent would be lost without a word: no operator here has a forward-mode derivative.
 constexpr const char *kNoTangent = "forward-mode derivatives are not supported, got a dual tensor";
@@ -194,6 +207,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         return {o.logp};
     }
     static variable_list backward(AutogradContext *ctx, variable_list up) {
+        not_traced();
         const auto kept = ctx->get_saved_variables();
         const Tensor &x = kept[0];
         Tensor grad;
@@ -212,6 +226,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 };
 
 py::object token_logprobs(const Tensor &x, const Tensor &tokens, const optional<Tensor> &mask, double temperature, bool entropy) {
+    not_traced();
     Tensor logp, ent;
     if (x.defined() && x.requires_grad() && at::GradMode::is_enabled()) {
         const variable_list o = TokenLogprobs::apply(x, tokens, mask, temperature, entropy);
@@ -281,6 +296,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         return {o.loss, o.logp, o.kl, o.clipped};
     }
     static variable_list backward(AutogradContext *ctx, variable_list up) {
+        not_traced();
         const auto kept = ctx->get_saved_variables();
         const Tensor &x = kept[0];
         Tensor grad;
@@ -338,6 +354,7 @@ Options options(const py::object &clip, double kl_coef, double temperature, cons
 py::tuple policy_loss(const Tensor &x, const Tensor &tokens, const Tensor &old, const Tensor &adv, const optional<Tensor> &mask,
                       const optional<Tensor> &ref, const py::object &clip, double kl_coef, double temperature,
                       const std::string &reduction, double scale, bool direct) {
+    not_traced();
     const Options opt = options(clip, kl_coef, temperature, reduction, scale, ref.has_value());
     if (!direct && x.requires_grad() && at::GradMode::is_enabled()) {
         const variable_list o = PolicyLoss::apply(x, tokens, old, adv, mask, ref, opt);
@@ -427,6 +444,7 @@ Tensor norm_of(const List &l, const Tensor &place) {
 }
 
 Tensor grad_norm(const py::object &grads, const py::object &current) {
+    not_traced();
     const List l = list_of("grads", grads);
     return norm_of(l, place_of(l, current));
 }
@@ -437,6 +455,7 @@ double checked_norm(double max_norm) {
 }
 
 Tensor clip_grad_norm(const py::object &grads, double max_norm, const py::object &current) {
+    not_traced();
     checked_norm(max_norm);
     const List l = list_of("grads", grads);
     const Tensor place = place_of(l, current), norm = norm_of(l, place);
@@ -450,6 +469,7 @@ Tensor clip_grad_norm(const py::object &grads, double max_norm, const py::object
 // dicts: weights, masters, exp_avg, exp_avg_sq, grads, of the same names in any order
 void adamw_step(const std::vector<py::dict> &dicts, int64_t step, double lr, double beta1, double beta2, double eps,
                 double weight_decay, const optional<Tensor> &norm, double max_norm) {
+    not_traced();
     static const char *const what[5] = {"weights", "masters", "exp_avg", "exp_avg_sq", "grads"};
     if (dicts.size() != 5) bad("adamw_step: expected five mappings");
     if (step < 1) bad("step counts from 1, got " + std::to_string(step));

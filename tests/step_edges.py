@@ -70,12 +70,10 @@ def _positions(dev, shape=(3,), vocab=9, seed=2):
 
 def _calls(x, y, f):
     """Every entry point by what it takes of a tensor: name -> (call of a tensor put in that place, the place's tensor)."""
-    state = lambda: [{"p": t.clone()} for t in (f, f, f, f, f)]  # noqa: E731
+    state = [t.clone() for t in (f, f, f, f, f)]
 
     def adamw(k, t):
-        s = state()
-        s[k]["p"] = t
-        crukx_sync.adamw_step(*s, step=1, lr=1e-3)
+        crukx_sync.adamw_step(*({"p": t if i == k else s} for i, s in enumerate(state)), step=1, lr=1e-3)
 
     return {
         "scores": (lambda t: crukx_sync.token_logprobs(t, y), x),
@@ -114,3 +112,49 @@ def forward_mode_derivatives_are_refused(dev):
         for r, u in ((crukx_sync.token_logprobs(leaf, y), up), (crukx_sync.policy_loss(leaf, y, f, f).loss, up[0])):
             with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
                 torch.autograd.grad(r, leaf, u)
+
+
+@edge
+def traced_calls_are_refused(dev):
+    """A trace would hold the allocation of the results and not the kernels that write them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, y, f = _positions(dev)
+    for call, at in _calls(x, y, f).values():
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (at.clone(),), check_trace=False)
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(call, tracing_mode=mode)(at.clone())
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(RuntimeError, match="cannot be traced"):
+            call(at.clone())
+        call(at.clone())
+    leaf = x.clone().requires_grad_()
+    for r in (crukx_sync.token_logprobs(leaf, y).sum(), crukx_sync.policy_loss(leaf, y, f, f).loss):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(lambda u: torch.autograd.grad(r, leaf, u, retain_graph=True)[0])(torch.ones_like(r))
+        assert torch.autograd.grad(r, leaf)[0].isfinite().all()
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda t: t + crukx_sync.grad_norm([]))(f)
+
+
+@edge
+def observed_calls_answer(dev):
+    """A dispatch mode that only looks on (a profiler's) changes nothing, and a compiled function calls the kernels between
+    its graphs."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class LooksOn(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, y, f = _positions(dev)
+    want = crukx_sync.token_logprobs(x, y)
+    leaf = x.clone().requires_grad_()
+    with LooksOn():
+        assert torch.equal(crukx_sync.token_logprobs(x, y), want)
+        grad, = torch.autograd.grad(crukx_sync.policy_loss(leaf, y, f, f + 1).loss, leaf)
+    assert torch.equal(grad, crukx_sync.policy_loss_grad(x, y, f, f + 1)[1])
+    compiled = torch.compile(lambda t: crukx_sync.token_logprobs(t * 2.0, y) + 1.0, backend="eager")
+    for t in (x, -x):
+        assert torch.equal(compiled(t), crukx_sync.token_logprobs(t * 2.0, y) + 1.0)
