@@ -60,6 +60,10 @@ void not_traced() {
     if (traced) throw std::runtime_error("the training step's calls cannot be traced");
 }
 
+// t with its data as they are meant: torch keeps some negations as a flag beside the data.  (Differentiable.)
+Tensor resolved(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+optional<Tensor> resolved(const optional<Tensor> &t) { return t.has_value() ? optional<Tensor>(resolved(*t)) : t; }
+
 // A dual tensor's tangent would be lost without a word: no operator here has a forward-mode derivative.
 constexpr const char *kNoTangent = "forward-mode derivatives are not supported, got a dual tensor";
 
@@ -211,8 +215,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         const auto kept = ctx->get_saved_variables();
         const Tensor &x = kept[0];
         Tensor grad;
-        const Tensor none;
-        const Tensor &up_logp = up[0], &up_entropy = up.size() > 1 ? up[1] : none;
+        const Tensor up_logp = resolved(up[0]), up_entropy = up.size() > 1 ? resolved(up[1]) : Tensor();
         if (up_logp.defined() || up_entropy.defined()) {
             const crx_logits in = logits_of(x, kept[1], kept[2], ctx->saved_data["temperature"].toDouble());
             const crx_positions a = floats_at("gradient", up_logp, x), h = floats_at("gradient", up_entropy, x);
@@ -225,8 +228,10 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     }
 };
 
-py::object token_logprobs(const Tensor &x, const Tensor &tokens, const optional<Tensor> &mask, double temperature, bool entropy) {
+py::object token_logprobs(const Tensor &x_, const Tensor &tokens_, const optional<Tensor> &mask_, double temperature, bool entropy) {
     not_traced();
+    const Tensor x = resolved(x_), tokens = resolved(tokens_);
+    const optional<Tensor> mask = resolved(mask_);
     Tensor logp, ent;
     if (x.defined() && x.requires_grad() && at::GradMode::is_enabled()) {
         const variable_list o = TokenLogprobs::apply(x, tokens, mask, temperature, entropy);
@@ -301,7 +306,8 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const Tensor &x = kept[0];
         Tensor grad;
         if (up[0].defined()) {
-            check_hip("gradient", up[0]);
+            const Tensor factor = resolved(up[0]);
+            check_hip("gradient", factor);
             const crx_logits in = logits_of(x, kept[1], kept[2], ctx->saved_data["temperature"].toDouble());
             const auto made = ctx->saved_data.find("grad");
             const bool first = made != ctx->saved_data.end();
@@ -313,7 +319,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
                 grad = new_grad(x);
             }
             const float *const stats = data(kept[3]);
-            call.done(g_api.policy_loss_grad(&in, stats, stats + 2 * in.seqs * in.tokens, data(up[0]), first ? 1 : 0,
+            call.done(g_api.policy_loss_grad(&in, stats, stats + 2 * in.seqs * in.tokens, data(factor), first ? 1 : 0,
                                              data<void>(grad), call.stream, call.err, sizeof call.err));
         }
         variable_list r(7);
@@ -351,11 +357,13 @@ Options options(const py::object &clip, double kl_coef, double temperature, cons
 }
 
 // (loss, logprobs, kl, clipped) with the loss's gradient by autograd, or (direct) the gradient as a fifth
-py::tuple policy_loss(const Tensor &x, const Tensor &tokens, const Tensor &old, const Tensor &adv, const optional<Tensor> &mask,
-                      const optional<Tensor> &ref, const py::object &clip, double kl_coef, double temperature,
+py::tuple policy_loss(const Tensor &x_, const Tensor &tokens_, const Tensor &old_, const Tensor &adv_, const optional<Tensor> &mask_,
+                      const optional<Tensor> &ref_, const py::object &clip, double kl_coef, double temperature,
                       const std::string &reduction, double scale, bool direct) {
     not_traced();
-    const Options opt = options(clip, kl_coef, temperature, reduction, scale, ref.has_value());
+    const Options opt = options(clip, kl_coef, temperature, reduction, scale, ref_.has_value());
+    const Tensor x = resolved(x_), tokens = resolved(tokens_), old = resolved(old_), adv = resolved(adv_);
+    const optional<Tensor> mask = resolved(mask_), ref = resolved(ref_);
     if (!direct && x.requires_grad() && at::GradMode::is_enabled()) {
         const variable_list o = PolicyLoss::apply(x, tokens, old, adv, mask, ref, opt);
         return py::make_tuple(o[0], o[1], o[2], o[3]);
@@ -468,7 +476,7 @@ Tensor clip_grad_norm(const py::object &grads, double max_norm, const py::object
 
 // dicts: weights, masters, exp_avg, exp_avg_sq, grads, of the same names in any order
 void adamw_step(const std::vector<py::dict> &dicts, int64_t step, double lr, double beta1, double beta2, double eps,
-                double weight_decay, const optional<Tensor> &norm, double max_norm) {
+                double weight_decay, const optional<Tensor> &norm_, double max_norm) {
     not_traced();
     static const char *const what[5] = {"weights", "masters", "exp_avg", "exp_avg_sq", "grads"};
     if (dicts.size() != 5) bad("adamw_step: expected five mappings");
@@ -478,6 +486,9 @@ void adamw_step(const std::vector<py::dict> &dicts, int64_t step, double lr, dou
     auto missing = [&](int k, PyObject *name) {
         bad(std::string(what[k]) + " and weights differ in tensor names" + (name ? ": " + py::str(name).cast<std::string>() : ""));
     };
+    auto negated = [&](int k, PyObject *name) {  // (a norm does not see signs, and a scale keeps them)
+        bad(std::string(what[k]) + " " + py::str(name).cast<std::string>() + ": the tensor is negated by a flag; pass its resolve_neg()");
+    };
     for (int k = 1; k < 5; ++k)
         if (dicts[k].size() != n) missing(k, nullptr);
     Py_ssize_t at[5] = {};
@@ -486,6 +497,7 @@ void adamw_step(const std::vector<py::dict> &dicts, int64_t step, double lr, dou
     while (PyDict_Next(dicts[0].ptr(), &at[0], &name, &weight)) {
         l[0].add(what[0], name, weight, false);
         const c10::TensorImpl *const w = l[0].t.back();
+        if (w->is_neg()) negated(0, name);
         for (int k = 1; k < 5; ++k) {
             PyObject *other, *item = nullptr;
             if (in_order[k]) in_order[k] = PyDict_Next(dicts[k].ptr(), &at[k], &other, &item) && (other == name || PyObject_RichCompareBool(other, name, Py_EQ) == 1);
@@ -494,16 +506,18 @@ void adamw_step(const std::vector<py::dict> &dicts, int64_t step, double lr, dou
             if (!item) missing(k, name);
             l[k].add(what[k], name, item, k < 4);
             const c10::TensorImpl *const o = l[k].t.back();
+            if (o->is_neg()) negated(k, name);
             if (o->sizes() != w->sizes()) bad(py::str(name).cast<std::string>() + ": " + what[k] + " and weights differ in shape");
             if (o->device() != w->device()) bad("all tensors must be on one device");
         }
     }
     crx_adamw a{lr, beta1, beta2, eps, weight_decay, (uint64_t)step, nullptr, 0.0};
-    if (norm.has_value()) {
-        check_hip("grad_norm", *norm);
-        if (norm->scalar_type() != at::kFloat || norm->numel() != 1) bad("grad_norm: expected one float32 value");
-        if (n && norm->device() != l[0].one.device()) bad("all tensors must be on one device");
-        a.norm = data(*norm);
+    const Tensor norm = resolved(or_none(norm_));
+    if (norm_.has_value()) {
+        check_hip("grad_norm", norm);
+        if (norm.scalar_type() != at::kFloat || norm.numel() != 1) bad("grad_norm: expected one float32 value");
+        if (n && norm.device() != l[0].one.device()) bad("all tensors must be on one device");
+        a.norm = data(norm);
         a.max_norm = checked_norm(max_norm);
     }
     if (!n) return;

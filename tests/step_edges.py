@@ -158,3 +158,44 @@ def observed_calls_answer(dev):
     compiled = torch.compile(lambda t: crukx_sync.token_logprobs(t * 2.0, y) + 1.0, backend="eager")
     for t in (x, -x):
         assert torch.equal(compiled(t), crukx_sync.token_logprobs(t * 2.0, y) + 1.0)
+
+
+@edge
+def lazily_negated_tensors_are_negated(dev):
+    """torch keeps some negations as a flag (the imaginary part of a conjugate), which the data do not show."""
+    x, y, f = _positions(dev, (2, 5))
+    g = _generator(3)
+    old, adv, rf = (torch.randn((2, 5), generator=g).to(dev) for _ in range(3))
+    neg = torch._neg_view
+    assert neg(x).is_neg() and torch.equal(neg(x), -x)
+    lp, h = crukx_sync.token_logprobs(neg(x), neg(-y), entropy=True)
+    assert all(torch.equal(a, b) for a, b in zip((lp, h), crukx_sync.token_logprobs(-x, y, entropy=True)))
+    opts = {"kl_coef": 0.1, "reduction": "sequence"}
+    want, want_grad = crukx_sync.policy_loss_grad(-x, y, old, adv, None, rf, **opts)
+    got, grad = crukx_sync.policy_loss_grad(neg(x), y, neg(-old), neg(-adv), None, neg(-rf), **opts)
+    assert torch.equal(got.loss, want.loss) and torch.equal(got.kl, want.kl) and torch.equal(grad, want_grad)
+    leaf = x.clone().requires_grad_()
+    loss = crukx_sync.policy_loss(neg(leaf), y, neg(-old), adv, None, rf, **opts).loss
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], -want_grad)
+    up = torch.randn((2, 5), generator=g).to(dev)  # upstream gradients
+    a, b = (torch.autograd.grad(crukx_sync.token_logprobs(leaf, y), leaf, u)[0] for u in (neg(up), -up))
+    assert torch.equal(a, b)
+    one = torch.ones((), device=dev)
+    a, b = (torch.autograd.grad(crukx_sync.policy_loss(leaf, y, old, adv).loss, leaf, u)[0] for u in (neg(-one * 3), one * 3))
+    assert torch.equal(a, b)
+    # lists: the norm does not see signs and clipping keeps them; a step would take them the wrong way round
+    t = up.clone()
+    assert torch.equal(crukx_sync.grad_norm([neg(t)]), crukx_sync.grad_norm([t]))
+    view = neg(t)
+    norm = crukx_sync.clip_grad_norm([view], 0.5)
+    ref.same(view, -up.double() * ref.factor(float(norm), 0.5), 4 * ref.U * up.abs().double())
+    s = [{"p": t.clone().abs()} for _ in range(5)]
+    for k in range(5):
+        with pytest.raises(ValueError, match="negat"):
+            crukx_sync.adamw_step(*({"p": neg(d["p"])} if i == k else d for i, d in enumerate(s)), step=1, lr=1e-3)
+        assert torch.equal(s[k]["p"], t.abs())
+    n = crukx_sync.grad_norm([t])
+    one, two = ([{"p": d["p"].clone()} for d in s] for _ in range(2))
+    crukx_sync.adamw_step(*one, step=1, lr=1e-3, grad_norm=n, max_norm=0.1)
+    crukx_sync.adamw_step(*two, step=1, lr=1e-3, grad_norm=neg(-n), max_norm=0.1)
+    assert all(torch.equal(a["p"], b["p"]) for a, b in zip(one, two))
