@@ -64,6 +64,13 @@ void not_traced() {
 Tensor resolved(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 optional<Tensor> resolved(const optional<Tensor> &t) { return t.has_value() ? optional<Tensor>(resolved(*t)) : t; }
 
+// An upstream gradient as data: torch may hand down one of nothing but zeros without any storage.
+Tensor upstream(const Tensor &t) { return t.defined() && t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : resolved(t); }
+
+// What holds no data itself (distributed, fake and zero tensors): a null address would read as an argument left out.
+constexpr const char *kNoStorage = "the tensor has no storage of its own";
+bool without_storage(const Tensor &t) { return t.numel() && !t.data_ptr(); }
+
 // A dual tensor's tangent would be lost without a word: no operator here has a forward-mode derivative.
 constexpr const char *kNoTangent = "forward-mode derivatives are not supported, got a dual tensor";
 
@@ -128,6 +135,7 @@ crx_positions positions(const char *name, const Tensor &t, const Tensor &like, a
         bad(std::string(name) + ": expected " + c10::toString(type) + (type == other ? "" : std::string(" or ") + c10::toString(other)) +
             ", got " + c10::toString(st));
     if (t.layout() != at::kStrided) bad(std::string(name) + ": expected a strided tensor");
+    if (without_storage(t)) bad(std::string(name) + ": " + kNoStorage);
     if (index_of(t) != index_of(like)) bad(std::string(name) + ": all tensors must be on one device");
     const auto want = like.sizes().slice(0, like.dim() - 1);
     bool fits = t.dim() == (int64_t)want.size();
@@ -149,6 +157,7 @@ crx_logits logits_of(const Tensor &x, const Tensor &tokens, const Tensor &mask, 
     const int32_t type = type_of(x);
     if (type < 0) bad(std::string("logits: expected bfloat16, float16 or float32, got ") + c10::toString(x.scalar_type()));
     if (x.layout() != at::kStrided) bad("logits: expected a strided tensor");
+    if (without_storage(x)) bad(std::string("logits: ") + kNoStorage);
     const int64_t dim = x.dim();
     if (dim != 2 && dim != 3)
         bad("logits: expected [tokens, vocabulary] or [sequences, tokens, vocabulary], got " + shape_of(x.sizes()));
@@ -215,7 +224,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         const auto kept = ctx->get_saved_variables();
         const Tensor &x = kept[0];
         Tensor grad;
-        const Tensor up_logp = resolved(up[0]), up_entropy = up.size() > 1 ? resolved(up[1]) : Tensor();
+        const Tensor up_logp = upstream(up[0]), up_entropy = up.size() > 1 ? upstream(up[1]) : Tensor();
         if (up_logp.defined() || up_entropy.defined()) {
             const crx_logits in = logits_of(x, kept[1], kept[2], ctx->saved_data["temperature"].toDouble());
             const crx_positions a = floats_at("gradient", up_logp, x), h = floats_at("gradient", up_entropy, x);
@@ -306,7 +315,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const Tensor &x = kept[0];
         Tensor grad;
         if (up[0].defined()) {
-            const Tensor factor = resolved(up[0]);
+            const Tensor factor = upstream(up[0]);
             check_hip("gradient", factor);
             const crx_logits in = logits_of(x, kept[1], kept[2], ctx->saved_data["temperature"].toDouble());
             const auto made = ctx->saved_data.find("grad");
@@ -410,6 +419,7 @@ struct List {
         if (impl->layout() != at::kStrided || !impl->is_contiguous()) fail("tensor must be contiguous");
         const int32_t k = type_of(v);
         if (k < 0 || (floats_only && k != CRX_F32)) fail(std::string("unexpected type ") + c10::toString(v.scalar_type()));
+        if (without_storage(v)) fail(kNoStorage);
         t.push_back(impl);
         ptr.push_back(v.data_ptr());
         numel.push_back((uint64_t)impl->numel());
@@ -516,6 +526,7 @@ void adamw_step(const std::vector<py::dict> &dicts, int64_t step, double lr, dou
     if (norm_.has_value()) {
         check_hip("grad_norm", norm);
         if (norm.scalar_type() != at::kFloat || norm.numel() != 1) bad("grad_norm: expected one float32 value");
+        if (without_storage(norm)) bad(std::string("grad_norm: ") + kNoStorage);
         if (n && norm.device() != l[0].one.device()) bad("all tensors must be on one device");
         a.norm = data(norm);
         a.max_norm = checked_norm(max_norm);

@@ -199,3 +199,45 @@ def lazily_negated_tensors_are_negated(dev):
     crukx_sync.adamw_step(*one, step=1, lr=1e-3, grad_norm=n, max_norm=0.1)
     crukx_sync.adamw_step(*two, step=1, lr=1e-3, grad_norm=neg(-n), max_norm=0.1)
     assert all(torch.equal(a["p"], b["p"]) for a, b in zip(one, two))
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor without storage of its own, as distributed and fake tensors are."""
+
+    @staticmethod
+    def __new__(cls, held):
+        t = torch.Tensor._make_wrapper_subclass(cls, held.shape, dtype=held.dtype, device=held.device, strides=held.stride())
+        t.held = held
+        return t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return func(*(a.held if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+
+
+@edge
+def tensors_without_storage_are_refused(dev):
+    """A mask or reference policy without data to read is refused, not left out."""
+    x, y, f = _positions(dev)
+    mask = torch.tensor([True, False, True], device=dev)
+    wrap = [_Wrapped, lambda t: torch._efficientzerotensor(t.shape, dtype=t.dtype, device=t.device)]
+    for w in wrap:
+        for call in (lambda t: crukx_sync.token_logprobs(x, y, t), lambda t: crukx_sync.policy_loss(x, y, f, f, t)):
+            call(mask)
+            with pytest.raises(ValueError, match="storage"):
+                call(w(mask))
+        with pytest.raises(ValueError, match="storage"):
+            crukx_sync.token_logprobs(x, w(y))
+        for name, (call, at) in _calls(x, y, f).items():
+            with pytest.raises(ValueError, match="storage"):
+                call(w(at))
+        with pytest.raises(ValueError, match="storage"):
+            crukx_sync.adamw_step(*({"p": f.clone()} for _ in range(5)), step=1, lr=1e-3, grad_norm=w(f[0]), max_norm=1.0)
+    # an upstream gradient of nothing is zeros
+    leaf = x.clone().requires_grad_()
+    zero = wrap[1]
+    for r, up in ((crukx_sync.token_logprobs(leaf, y), zero(f)), (crukx_sync.policy_loss(leaf, y, f, f + 1).loss, zero(f[0]))):
+        assert not torch.autograd.grad(r, leaf, up)[0].any()
+    empty = x[:0].clone().requires_grad_()  # no elements: nothing to read either
+    crukx_sync.policy_loss(empty, y[:0], f[:0], f[:0], mask[:0], f[:0]).loss.backward()
+    assert crukx_sync.token_logprobs(empty, y[:0], mask[:0]).shape == (0,) and empty.grad.shape == (0, 9)
