@@ -610,7 +610,19 @@ struct Token {
     float loss, kl, cut, slope;  // slope: the loss's derivative by the log probability
 };
 
-// The position's loss.  The KL term e^d - 1 - d loses its leading digits where d is small: there, its series.
+// e^d - 1 - d.  The difference loses leading digits where d is small (five bits at 1/16): below 1, its series, d^2 times the
+// sum of d^n / (n + 2)!, of which eleven terms are kept (the twelfth is under 2^-30 of the sum).
+__device__ __forceinline__ float kl_term(float d, float expm1_d) {
+    if (!(fabsf(d) < 1.0f)) return expm1_d - d;
+    constexpr float over[] = {0.5f, 1.0f / 6, 1.0f / 24, 1.0f / 120, 1.0f / 720, 1.0f / 5040, 1.0f / 40320, 1.0f / 362880,
+                              1.0f / 3628800, 1.0f / 39916800, 1.0f / 479001600};
+    float p = over[10];
+#pragma unroll
+    for (int k = 9; k >= 0; --k) p = fmaf(d, p, over[k]);
+    return d * d * p;
+}
+
+// The position's loss.
 __device__ __forceinline__ Token token_loss(const PolicyIn &p, const Row &r, Two logp) {
     const float A = value_at(p.adv, r), ratio = expf((logp.hi - value_at(p.old, r)) + logp.lo);
     const float held = fminf(fmaxf(ratio, p.low), p.high);
@@ -624,9 +636,7 @@ __device__ __forceinline__ Token token_loss(const PolicyIn &p, const Row &r, Two
     o.kl = 0.0f;
     if (p.ref.p) {
         const float d = (value_at(p.ref, r) - logp.hi) - logp.lo, g = expm1f(d);
-        o.kl = fabsf(d) < 0.0625f
-                   ? d * d * (0.5f + d * (1.0f / 6 + d * (1.0f / 24 + d * (1.0f / 120 + d * (1.0f / 720)))))
-                   : g - d;
+        o.kl = kl_term(d, g);
         o.loss += p.kl * o.kl;
         o.slope -= p.kl * g;
     }

@@ -241,3 +241,25 @@ def tensors_without_storage_are_refused(dev):
     empty = x[:0].clone().requires_grad_()  # no elements: nothing to read either
     crukx_sync.policy_loss(empty, y[:0], f[:0], f[:0], mask[:0], f[:0]).loss.backward()
     assert crukx_sync.token_logprobs(empty, y[:0], mask[:0]).shape == (0,) and empty.grad.shape == (0, 9)
+
+
+# ------------------------------------------------------------------ values
+
+@edge
+def kl_terms_of_every_size(dev):
+    """exp(d) - 1 - d, position by position.  One id in the vocabulary: its log probability is exactly 0, so d is the
+    reference's value itself, and with an advantage of 0 the loss is the KL term alone.
+
+    The term is a product of d^2 and a sum whose parts add up to at least a third of their absolute sum (|d| < 1), or a
+    difference that leaves at least a third of what is subtracted (beyond), each from operations of one or two roundings:
+    16 u bound it."""
+    x, y = torch.zeros((1, 1), device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    zero = torch.zeros(1, device=dev)
+    sizes = [1e-30, 1e-12, 1e-6, 1e-3, 0.03, 0.0624, 0.0626, 0.07, 0.09, 0.12, 0.2, 0.249, 0.251, 0.4, 0.49, 0.51, 0.7, 0.99, 1.01, 1.5, 3.0, 20.0, 80.0]
+    for d in [s * a for a in sizes for s in (1, -1)] + [0.0]:
+        at = torch.tensor([d], device=dev)
+        out, _ = crukx_sync.policy_loss_grad(x, y, zero, zero, None, at, kl_coef=1.0, reduction="sum")
+        v = at.cpu().double()
+        want = (v * v / 2 * (1 + v / 3) if abs(d) < 1e-3 else torch.special.expm1(v) - v).sum()
+        tol = 16 * ref.U * float(want) + 2.0 ** -149
+        assert abs(float(out.kl) - float(want)) <= tol and abs(float(out.loss) - float(want)) <= tol, (d, float(out.kl), float(want))
