@@ -16,8 +16,9 @@ namespace crx {
 namespace {
 
 constexpr float kLn2 = 0.69314718055994531f;
-// below every log2-scaled difference that matters, and finite: stands for -inf where it is multiplied
-constexpr float kFloor = -1e30f;
+// a log2-scaled difference whose power of 2 is 0, as that of everything below it: stands for -inf where it is multiplied
+// (and no larger, so that its products with an upstream gradient stay finite: they are multiplied by that 0)
+constexpr float kFloor = -256.0f;
 
 __device__ __forceinline__ uint32_t wave_lane() { return threadIdx.x & 63u; }
 // (the generic min template of the HIP headers goes through double precision)

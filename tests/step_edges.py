@@ -263,3 +263,23 @@ def kl_terms_of_every_size(dev):
         want = (v * v / 2 * (1 + v / 3) if abs(d) < 1e-3 else torch.special.expm1(v) - v).sum()
         tol = 16 * ref.U * float(want) + 2.0 ** -149
         assert abs(float(out.kl) - float(want)) <= tol and abs(float(out.loss) - float(want)) <= tol, (d, float(out.kl), float(want))
+
+
+@edge
+def entropy_gradients_of_any_size_pass_impossible_ids_by(dev):
+    """An id without probability has no gradient, however large the upstream one (a loss scale): 0, not NaN."""
+    g = _generator(5)
+    for dtype, rows, vocab in ((torch.float32, 2, 515), (torch.bfloat16, 300, 515)):
+        x = (torch.randn((rows, vocab), generator=g) * 2).to(dtype).to(dev)
+        x[:, 400:] = -float("inf")
+        x[0, 17] = torch.finfo(dtype).min
+        y = torch.randint(0, 400, (rows,), generator=g).to(dev)
+        for up in (1.0, 1e12, 1e30):
+            leaf = x.clone().requires_grad_()
+            lp, h = crukx_sync.token_logprobs(leaf, y, entropy=True)
+            u = torch.full((rows,), up, device=dev)
+            for outs, ups, a in (([h], [u], None), ([lp, h], [u, u], u)):
+                got, = torch.autograd.grad(outs, leaf, ups, retain_graph=True)
+                assert not got[:, 400:].any() and not got[0, 17].any()
+                want = ref.scores_grad(x, y, a, u)
+                ref.check_grad(got, want, u.double() * (2 + 2 * 8), vocab)
