@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <limits>
 #include <new>
 #include <string>
 
@@ -91,8 +92,10 @@ bool rows_in(const crx_logits *x, RowsIn &o) {
     o.ids_st = x->ids.stride_token;
     o.id_bytes = x->id_bytes;
     o.mask = at<uint8_t>(x->mask);
-    o.c = (float)(1.4426950408889634 / x->temperature);
-    o.inv_temp = (float)(1.0 / x->temperature);
+    // not 0, whatever the temperature: -inf times it has to stay -inf
+    const auto inverse = [&](double a) { return std::max((float)(a / x->temperature), std::numeric_limits<float>::denorm_min()); };
+    o.c = inverse(1.4426950408889634);
+    o.inv_temp = inverse(1.0);
     o.inv_temp_lo = (float)(1.0 / x->temperature - (double)o.inv_temp);
     if (!std::isfinite(o.c)) throw Invalid("temperature is too small for 32-bit arithmetic");
     return true;

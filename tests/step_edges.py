@@ -283,3 +283,18 @@ def entropy_gradients_of_any_size_pass_impossible_ids_by(dev):
                 assert not got[:, 400:].any() and not got[0, 17].any()
                 want = ref.scores_grad(x, y, a, u)
                 ref.check_grad(got, want, u.double() * (2 + 2 * 8), vocab)
+
+
+@edge
+def temperatures_up_to_the_largest(dev):
+    """The distribution becomes uniform over the ids that have a probability, and stays one."""
+    x, y, f = _positions(dev, (4,), 20)
+    x[:, 13:] = -float("inf")
+    y %= 13
+    for t in (1e6, 1e30, 1e38, 1e44, 1e46, 1e300, 1.7e308):
+        lp, h = crukx_sync.token_logprobs(x, y, temperature=t, entropy=True)
+        ref.check_scores(x, y, None, t, lp, h)
+        out, grad = crukx_sync.policy_loss_grad(x, y, f - 2, f + 1, temperature=t)
+        ref.check_policy(x, y, f - 2, f + 1, None, None, {"temperature": t}, out, grad if t <= 1e38 else None)
+        if t > 1e38:  # smaller than any 32-bit number says to a place
+            assert grad.isfinite().all() and float(grad.abs().max()) <= 1e-43
