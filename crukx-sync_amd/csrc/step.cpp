@@ -29,6 +29,13 @@ void check_aligned(const void *p, uint32_t bytes, const char *what) {
     if (reinterpret_cast<uintptr_t>(p) % bytes) throw Invalid(std::string(what) + ": data must be aligned to its elements");
 }
 
+// Floats (absent ones are at 0), and pairs of them, which are read and written 8 bytes at a time.
+template <typename... P>
+void check_floats(const P *...p) {
+    for (const void *q : {static_cast<const void *>(p)...}) check_aligned(q, 4, "float data");
+}
+void check_stats(const float *p) { check_aligned(p, 8, "statistics"); }
+
 void launched() {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) throw DeviceError(std::string("kernel launch: ") + hipGetErrorString(e));
@@ -100,7 +107,6 @@ bool rows_in(const crx_logits *x, RowsIn &o) {
     if (!std::isfinite(o.c)) throw Invalid("temperature is too small for 32-bit arithmetic");
     return true;
 }
-
 
 uint32_t units_of(uint64_t elements) { return (uint32_t)((elements + kUnit - 1) / kUnit); }
 
@@ -179,6 +185,8 @@ int32_t crx_token_logprobs(const crx_logits *x, float *logprobs, float *entropy,
         RowsIn in;
         if (!rows_in(x, in)) return;
         if (!logprobs || !scratch) throw Invalid("token_logprobs: no place for the results");
+        check_floats(logprobs, entropy, scratch);
+        check_stats(stats);
         Parts parts = parts_of(in.rows, in.vocab);
         parts.stat = static_cast<float *>(scratch);
         launch_score(in, parts, ScoreOut{logprobs, entropy, reinterpret_cast<float2 *>(stats)}, x->dtype,
@@ -201,6 +209,8 @@ int32_t crx_token_logprobs_grad(const crx_logits *x, const float *stats, const f
         g.grad = grad;
         if (!stats || !grad || (g.up_entropy.p && !entropy)) throw Invalid("token_logprobs: no statistics or no place for the gradient");
         check_aligned(grad, size_of(x->dtype), "gradient");
+        check_floats(entropy, g.up_logp.p, g.up_entropy.p);
+        check_stats(stats);
         launch_rows_grad(in, g, x->dtype, static_cast<hipStream_t>(stream));
         launched();
     });
@@ -216,6 +226,9 @@ int32_t crx_policy_loss(const crx_logits *x, const crx_policy *p, float *loss, f
         if (p->reduction != kMeanToken && p->reduction != kMeanSequence && p->reduction != kSum)
             throw Invalid("policy_loss: unknown reduction");
         if (!(p->clip_low >= 0.0) || !(p->clip_high >= 0.0)) throw Invalid("policy_loss: the clip range must not be negative");
+        check_floats(loss, kl, clipped, logprobs, slope, scratch);
+        check_floats(p->old.p, p->advantages.p, p->ref.p);
+        check_stats(stats);
         if (p->kl_coef != 0.0 && !p->ref.p && any) throw Invalid("policy_loss: a KL coefficient needs reference log probabilities");
         if (!any) {
             launch_policy_sums(nullptr, 0, 1.0f, loss, kl, clipped, s);
@@ -255,6 +268,8 @@ int32_t crx_policy_loss_grad(const crx_logits *x, const float *stats, const floa
         if (!rows_in(x, in)) return;
         if (!stats || !slope || !upstream || !grad) throw Invalid("policy_loss: no statistics or no place for the gradient");
         check_aligned(grad, size_of(x->dtype), "gradient");
+        check_floats(slope, upstream);
+        check_stats(stats);
         GradIn g{};
         g.stats = reinterpret_cast<const float2 *>(stats);
         g.slope = slope;
@@ -276,6 +291,7 @@ int32_t crx_grad_norm(int32_t n, const void *const *grads, const uint64_t *numel
         const hipStream_t s = static_cast<hipStream_t>(stream);
         if (!norm || !scratch) throw Invalid("grad_norm: missing arguments");
         check_aligned(scratch, 8, "scratch");
+        check_floats(norm);
         double *const partial = static_cast<double *>(scratch);
         uint32_t used = 0;  // partial sums written so far: later launches add to them
         over_tensors(n, const_cast<void *const *>(grads), numels, dtypes, kNormUnits, [&](const NormList &l, int type, bool keep) {
@@ -293,6 +309,7 @@ int32_t crx_clip_grads(int32_t n, void *const *grads, const uint64_t *numels, co
     return guarded_step(err, errlen, [&] {
         if (!norm) throw Invalid("clip_grads: missing arguments");
         if (!(max_norm >= 0.0)) throw Invalid("max_norm must not be negative");
+        check_floats(norm);
         over_tensors(n, grads, numels, dtypes, kClipUnits, [&](const NormList &l, int type, bool keep) {
             launch_clip(l, type, norm, (float)max_norm, keep, blocks_for(l.first[l.count], kClipShare), static_cast<hipStream_t>(stream));
         });
@@ -311,6 +328,7 @@ int32_t crx_adamw_step(int32_t n, void *const *weights, float *const *masters, f
         if (!(a->lr >= 0.0) || !(a->eps >= 0.0) || !(a->weight_decay >= 0.0)) throw Invalid("adamw: lr, eps and weight_decay must not be negative");
         if (!(a->beta1 >= 0.0 && a->beta1 < 1.0) || !(a->beta2 >= 0.0 && a->beta2 < 1.0)) throw Invalid("adamw: betas must be in [0, 1)");
         if (a->norm && !(a->max_norm >= 0.0)) throw Invalid("max_norm must not be negative");
+        check_floats(a->norm);
         for (int32_t i = 0; i < n; ++i) {
             check_type(weight_dtypes[i], "weights");
             check_type(grad_dtypes[i], "gradients");

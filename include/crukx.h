@@ -266,7 +266,8 @@ typedef struct crx_logits {
 uint64_t crx_rows_scratch(uint64_t seqs, uint64_t tokens, uint64_t vocab);
 
 /* logprobs[seqs*tokens]: log softmax(x / temperature) at the sampled token; entropy (or NULL): of the whole
- * distribution, in nats; stats (or NULL): what crx_token_logprobs_grad needs, two floats per position. */
+ * distribution, in nats; stats (or NULL): what crx_token_logprobs_grad needs, two floats per position, aligned to
+ * 8 bytes (floats elsewhere to 4, tensors to their elements: CRX_INVALID otherwise). */
 int32_t crx_token_logprobs(const crx_logits *x, float *logprobs, float *entropy, float *stats, void *scratch,
                            void *stream, char *err, uint64_t errlen);
 /* grad[seqs*tokens*vocab], of x's type: the gradient of sum(up_logprobs * logprobs + up_entropy * entropy)
