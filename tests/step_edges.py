@@ -7,7 +7,9 @@ import pytest
 import torch
 
 import crukx_sync
+import step_cases as cases
 import step_reference as ref
+import step_rows as rows
 
 EDGES = {}
 
@@ -298,3 +300,56 @@ def temperatures_up_to_the_largest(dev):
         ref.check_policy(x, y, f - 2, f + 1, None, None, {"temperature": t}, out, grad if t <= 1e38 else None)
         if t > 1e38:  # smaller than any 32-bit number says to a place
             assert grad.isfinite().all() and float(grad.abs().max()) <= 1e-43
+
+
+# ------------------------------------------------------------------ gradients, element by element
+
+def _shapes(dev):
+    """Rows cut into parts, rows of a wavefront, of 256 threads, of 1024 that share a CU and of 1024 that have one."""
+    if dev == "cpu":
+        return [((3, 4, 9), 1.0), ((3, 4, 130), 1.0), ((2, 2, 4099), 1.0), ((260, 515), 0.7), ((257, 8200), 0.03), ((256, 40007), 0.01)]
+    return [((3, 4, v), 0.8) for v in (1, 2, 7, 8, 9, 63, 257, 1000, 4096, 4097, 20011, 65537, 151936)] + \
+        [((300, 515), 0.8), ((20, 15, 4099), 0.8), ((270, 8200), 0.8), ((260, 40007), 0.5), ((260, 115_003), 0.4), ((2, 130, 152_064), 0.3)]
+
+
+def _row_cases(dev, dtype, seed):
+    for shape, share in _shapes(dev):
+        x, y = cases.logits(shape, dtype, seed + shape[-1], dev)
+        old, rf, adv = cases.policies(x, y, seed, device=dev)
+        mask = cases.mask_of(shape[:-1], seed, dev, share)
+        mask.view(-1)[0] = True
+        yield x, y, old, rf, adv, mask
+        if shape[-1] in (130, 257, 8200, 115_003):  # the same at other alignments than the gradient's
+            wide = torch.full((*shape[:-1], shape[-1] + 6), float("nan"), dtype=x.dtype, device=dev)
+            wide[..., 5:shape[-1] + 5] = x
+            yield wide[..., 5:shape[-1] + 5], y, old, rf, adv, mask
+
+
+def _loss_scale(dtype):
+    return 1024.0 if dtype == "fp16" else 1.0  # without one fp16 holds little of a small gradient
+
+
+def _policy_rows(dev, dtype):
+    for k, (x, y, old, rf, adv, mask) in enumerate(_row_cases(dev, dtype, 3)):
+        opts = {"clip": (0.2, 0.28), "kl_coef": 0.05, "reduction": ("sequence", "token", "sum")[k % 3], "scale": _loss_scale(dtype)}
+        _, grad = crukx_sync.policy_loss_grad(x, y, old, adv, mask, rf, **opts)
+        rows.check_policy_gradient(grad, x, y, old, adv, mask, rf, **opts)
+
+
+def _score_rows(dev, dtype):
+    g = _generator(4)
+    for k, (x, y, _, _, _, mask) in enumerate(_row_cases(dev, dtype, 5)):
+        up, uh = ((torch.randn(y.shape, generator=g) * _loss_scale(dtype)).to(dev) for _ in range(2))
+        leaf = x.detach().requires_grad_()
+        if k % 2:
+            lp, h = crukx_sync.token_logprobs(leaf, y, mask, temperature=0.8, entropy=True)
+            got, = torch.autograd.grad([lp, h], leaf, [up, uh])
+        else:
+            uh = None
+            got, = torch.autograd.grad(crukx_sync.token_logprobs(leaf, y, mask, temperature=0.8), leaf, up)
+        rows.check_score_gradient(got, x, y, up, uh, mask, 0.8)
+
+
+for _dtype in sorted(cases.TYPES):
+    EDGES[f"policy_gradients_row_by_row_{_dtype}"] = lambda dev, t=_dtype: _policy_rows(dev, t)
+    EDGES[f"score_gradients_row_by_row_{_dtype}"] = lambda dev, t=_dtype: _score_rows(dev, t)
