@@ -353,3 +353,83 @@ def _score_rows(dev, dtype):
 for _dtype in sorted(cases.TYPES):
     EDGES[f"policy_gradients_row_by_row_{_dtype}"] = lambda dev, t=_dtype: _policy_rows(dev, t)
     EDGES[f"score_gradients_row_by_row_{_dtype}"] = lambda dev, t=_dtype: _score_rows(dev, t)
+
+
+@edge
+def upstream_factors_over_many_parts(dev):
+    """A loss divided by a number of accumulations: the first backward pass writes the gradient anew, its workgroups each for
+    several parts of rows (more parts than workgroups are launched), and equals the loss made with that scale."""
+    rows_, vocab, share = (700, 40_007, 0.9) if dev != "cpu" else (2100, 40, 0.9)  # 700 x 5 parts, 2100 x 1; 2048 workgroups
+    x, y = cases.logits((rows_, vocab), "bf16", 9, dev)
+    old, rf, adv = cases.policies(x, y, 9, device=dev)
+    mask = cases.mask_of((rows_,), 9, dev, share)
+    opts = {"clip": (0.2, 0.28), "kl_coef": 0.05}
+    for factor in (0.5, -3.0):
+        leaf = x.detach().requires_grad_()
+        loss = crukx_sync.policy_loss(leaf, y, old, adv, mask, rf, **opts).loss * factor
+        got, = torch.autograd.grad(loss, leaf)
+        rows.check_policy_gradient(got, x, y, old, adv, mask, rf, scale=factor, **opts)
+
+
+@edge
+def gradients_with_a_graph_have_the_same_values(dev):
+    """create_graph hands out the same gradient, once from the loss's forward call and anew after that."""
+    x, y, f = _positions(dev, (2, 5), 33)
+    leaf = x.clone().requires_grad_()
+    want = crukx_sync.policy_loss_grad(x, y, f - 2, f + 1)[1]
+    loss = crukx_sync.policy_loss(leaf, y, f - 2, f + 1).loss
+    for _ in range(2):
+        got, = torch.autograd.grad(loss, leaf, create_graph=True)
+        assert got.requires_grad and torch.equal(got.detach(), want) and bool(want.any())
+    scores = crukx_sync.token_logprobs(leaf, y).sum()
+    plain, = torch.autograd.grad(scores, leaf, retain_graph=True)
+    got, = torch.autograd.grad(scores, leaf, create_graph=True)
+    assert got.requires_grad and torch.equal(got.detach(), plain) and bool(plain.any())
+
+
+PAIRS = [(w, g) for w in sorted(cases.TYPES) for g in sorted(cases.TYPES)]
+
+
+def _check_step(before, after, k, c, step=5, lr=1e-3, wd=0.1):
+    w0, m0, v0, g0 = (d[k] for d in before[1:])
+    a, b, d = ref.adamw(w0, m0, v0, g0, step, lr, (0.9, 0.999), 1e-8, wd, c)
+    g = g0.double().abs() * c
+    ref.same(after[2][k], b, 8 * ref.U * (m0.abs().double() + g), "exp_avg")
+    ref.same(after[3][k], d, 8 * ref.U * (v0.double() + g * g), "exp_avg_sq")
+    size = lr / (1 - 0.9 ** step) / ((d / (1 - 0.999 ** step)).sqrt() + 1e-8) * (m0.abs().double() + g)
+    ref.same(after[1][k], a, 4 * ref.U * w0.abs().double() + 32 * ref.U * size, "masters")
+    assert torch.equal(after[0][k], after[1][k].to(after[0][k].dtype)), "weights"
+    assert torch.equal(after[4][k], before[4][k]), "gradients"
+
+
+@edge
+def adamw_of_every_pair_of_types_and_of_all_in_one_call(dev):
+    """Nine pairs of weight and gradient types alone; and one call with all of them, in an order that changes the pair from
+    tensor to tensor, over flat buffers where the neighbours of a tensor have another pair (and some the same)."""
+    sizes = [5, 1024, 1, 2049, 7, 300, 0, 4099, 64]
+    g = _generator(8)
+
+    def flat(types, scale, positive=False):
+        """Tensors of `sizes`, type by type, those of one type one behind another in one buffer."""
+        bufs = {t: (torch.randn(sum(sizes), generator=g) * scale).abs_() if positive else torch.randn(sum(sizes), generator=g) * scale
+                for t in cases.TYPES}
+        bufs = {t: b.to(cases.TYPES[t]).to(dev) for t, b in bufs.items()}
+        out, at = {}, dict.fromkeys(bufs, 0)
+        for k, (n, t) in enumerate(zip(sizes, types)):
+            out[f"p{k}"] = bufs[t][at[t]:at[t] + n]
+            at[t] += n
+        return out
+
+    lists = [([w] * 9, [q] * 9) for w, q in PAIRS]
+    lists.append(([w for w, _ in PAIRS], [q for _, q in PAIRS]))
+    lists.append((["bf16", "bf16", "fp32", "bf16", "bf16", "fp16", "bf16", "bf16", "fp32"],
+                  ["bf16", "bf16", "bf16", "fp32", "bf16", "bf16", "bf16", "bf16", "fp16"]))
+    for wtypes, gtypes in lists:
+        floats = ["fp32"] * 9
+        s = [flat(wtypes, 1.0), flat(floats, 1e-2), flat(floats, 1e-2), flat(floats, 1e-4, True), flat(gtypes, 1.0)]
+        before = [{k: t.clone() for k, t in d.items()} for d in s]
+        norm = crukx_sync.grad_norm(s[4])
+        ref.same(norm, ref.norm(list(s[4].values())), 2 * ref.U * float(norm), "norm")
+        crukx_sync.adamw_step(*s, step=5, lr=1e-3, weight_decay=0.1, grad_norm=norm, max_norm=1.0)
+        for k in s[0]:
+            _check_step(before, s, k, ref.factor(float(norm), 1.0))
