@@ -765,33 +765,23 @@ __device__ __forceinline__ void for_share(const L &l, uint32_t i, uint32_t n, F 
     }
 }
 
-// Loads a thread has in flight in the passes over lists.  The norm's 64-bit sums leave few registers: with one load eight
-// wavefronts fit a SIMD, which hides more (7.6e9 bf16 gradients 2216 us; two 2293, four 2298).
-constexpr uint32_t kNormLoads = 1, kClipLoads = 2;
+// Loads a thread has in flight in the passes over lists.  The norm has one: its 64-bit sums leave few registers, and so eight
+// wavefronts fit a SIMD, which hides more (7.6e9 bf16 gradients 2216 us; with two loads 2293, with four 2298).
+constexpr uint32_t kClipLoads = 2;
 
 template <typename T, bool KEEP>
 __device__ __forceinline__ double squares(const uint8_t *p, uint64_t lo, uint64_t hi) {
     constexpr uint32_t N = Lane<T>::N, STEP = 256 * N;
     double n = 0.0;
     float f[N];
-    uint32_t w[kNormLoads][4];
+    uint32_t w[4];
     const Span<T> sp(p, lo, hi);
     const uint64_t body = sp.first + sp.vectors * N;
-    uint64_t i = sp.first + threadIdx.x * N;
-    auto add = [&](const uint32_t *v) {
-        Lane<T>::unpack(v, f);
+    for (uint64_t i = sp.first + threadIdx.x * N; i < body; i += STEP) {
+        if (KEEP) load16(p + i * sizeof(T), w);
+        else load16_stream(p + i * sizeof(T), w);
+        Lane<T>::unpack(w, f);
         for (uint32_t k = 0; k < N; ++k) n += (double)f[k] * (double)f[k];
-    };
-    for (; i + (kNormLoads - 1) * STEP < body; i += kNormLoads * STEP) {
-        for (uint32_t u = 0; u < kNormLoads; ++u) {
-            if (KEEP) load16(p + (i + u * STEP) * sizeof(T), w[u]);
-            else load16_stream(p + (i + u * STEP) * sizeof(T), w[u]);
-        }
-        for (uint32_t u = 0; u < kNormLoads; ++u) add(w[u]);
-    }
-    for (; i < body; i += STEP) {
-        load16(p + i * sizeof(T), w[0]);
-        add(w[0]);
     }
     if (threadIdx.x < sp.edges) {
         const double v = (double)Lane<T>::get(p + sp.edge(threadIdx.x) * sizeof(T));
