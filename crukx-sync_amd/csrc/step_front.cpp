@@ -69,7 +69,7 @@ Tensor upstream(const Tensor &t) { return t.defined() && t._is_zerotensor() ? at
 
 // What holds no data itself (distributed, fake and zero tensors): a null address would read as an argument left out.
 constexpr const char *kNoStorage = "the tensor has no storage of its own";
-bool without_storage(const Tensor &t) { return t.numel() && !t.data_ptr(); }
+bool without_storage(const Tensor &t) { return !t.data_ptr() && t.numel(); }
 
 // A dual tensor's tangent would be lost without a word: no operator here has a forward-mode derivative.
 constexpr const char *kNoTangent = "forward-mode derivatives are not supported, got a dual tensor";
@@ -419,10 +419,12 @@ struct List {
         if (impl->layout() != at::kStrided || !impl->is_contiguous()) fail("tensor must be contiguous");
         const int32_t k = type_of(v);
         if (k < 0 || (floats_only && k != CRX_F32)) fail(std::string("unexpected type ") + c10::toString(v.scalar_type()));
-        if (without_storage(v)) fail(kNoStorage);
+        void *const at = v.data_ptr();
+        const uint64_t n = (uint64_t)impl->numel();
+        if (!at && n) fail(kNoStorage);
         t.push_back(impl);
-        ptr.push_back(v.data_ptr());
-        numel.push_back((uint64_t)impl->numel());
+        ptr.push_back(at);
+        numel.push_back(n);
         type.push_back(k);
     }
 };
