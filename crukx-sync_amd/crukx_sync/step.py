@@ -123,7 +123,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.
     that have an unmasked position of the sequence's mean ("sequence"), or their sum ("sum"; 2-d logits are one
     sequence).  Without any unmasked position it is 0.  Differentiable by the logits only; at a clip limit itself
     a position counts as not clipped.  logits, tokens and mask as in token_logprobs; old_logprobs, advantages and
-    ref_logprobs float32, of the positions' shape or broadcast to it."""
+    ref_logprobs float32, with as many dimensions as tokens, each of its size or of size 1 (advantages of
+    [sequences, 1]: one for all tokens of a sequence)."""
     return PolicyLoss(*_policy(logits, tokens, old_logprobs, advantages, mask, ref_logprobs, clip, kl_coef, temperature,
                                reduction, scale, False))
 
@@ -148,13 +149,15 @@ def _items(tensors):
 
 def grad_norm(grads) -> torch.Tensor:
     """The 2-norm of all elements of all gradients together, a 0-d float32 tensor on their device.  grads: a mapping
-    or a sequence of contiguous bf16, fp16 or fp32 tensors.  Squares are summed in 64 bits."""
+    or a sequence of contiguous bf16, fp16 or fp32 tensors.  Squares are summed in 64 bits.  The norm itself carries no
+    gradient, also where the tensors require one."""
     return (_front or _load()).grad_norm(_items(grads), torch.cuda.current_device)
 
 
 def clip_grad_norm(grads, max_norm: float) -> torch.Tensor:
     """Scales every gradient, in place, by min(1, max_norm / (norm + 1e-6)), and returns the norm that they had
-    (grad_norm).  An infinite norm scales by 0, a NaN makes every gradient NaN."""
+    (grad_norm).  An infinite norm scales by 0, a NaN makes every gradient NaN.  No two tensors may overlap: a tensor
+    listed twice counts twice in the norm and may be scaled twice."""
     return (_front or _load()).clip_grad_norm(_items(grads), max_norm, torch.cuda.current_device)
 
 

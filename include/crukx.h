@@ -309,7 +309,7 @@ uint64_t crx_norm_scratch(void);
 int32_t crx_grad_norm(int32_t n, const void *const *grads, const uint64_t *numels, const int32_t *dtypes, float *norm,
                       void *scratch, void *stream, char *err, uint64_t errlen);
 /* Every gradient times c = min(1, max_norm / (*norm + 1e-6)), in place, rounded once; nothing is written
- * where c is 1. */
+ * where c is 1.  No two tensors may overlap. */
 int32_t crx_clip_grads(int32_t n, void *const *grads, const uint64_t *numels, const int32_t *dtypes, const float *norm,
                        double max_norm, void *stream, char *err, uint64_t errlen);
 
@@ -321,7 +321,8 @@ typedef struct crx_adamw {
 } crx_adamw;
 
 /* One AdamW step (decoupled decay) of n tensors, in place: fp32 masters and moments, gradients of any type,
- * and the weights (bf16, fp16 or fp32), which become the new masters rounded to nearest. */
+ * and the weights (bf16, fp16 or fp32), which become the new masters rounded to nearest.  No two tensors may
+ * overlap. */
 int32_t crx_adamw_step(int32_t n, void *const *weights, float *const *masters, float *const *exp_avg,
                        float *const *exp_avg_sq, const void *const *grads, const uint64_t *numels,
                        const int32_t *weight_dtypes, const int32_t *grad_dtypes, const crx_adamw *a, void *stream,
