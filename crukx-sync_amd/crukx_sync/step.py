@@ -170,8 +170,8 @@ def adamw_step(weights: Mapping[str, torch.Tensor], masters: Mapping[str, torch.
         g = c * grad;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
         w = w (1 - lr * weight_decay) - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps)
 
-    w, m and v are the float32 masters, exp_avg and exp_avg_sq; the weights (bf16, fp16 or fp32: what
-    encode_update takes) become the new masters, rounded to nearest even.  With grad_norm (a 0-d float32 tensor
+    w, m and v are the float32 masters, exp_avg and exp_avg_sq; the weights (bf16, which encode_update
+    takes, fp16 or fp32) become the new masters, rounded to nearest even.  With grad_norm (a 0-d float32 tensor
     from grad_norm(), or one reduced over ranks) and max_norm the gradients are clipped on the way, without being
     written: c = min(1, max_norm / (grad_norm + 1e-6)).  `step` counts from 1.  All mappings hold the same names
     and shapes; no two tensors may overlap."""

@@ -101,9 +101,9 @@ constexpr uint32_t kNormBlocks = 2048;  // workgroups of the norm's pass, most: 
 constexpr uint32_t kNormShare = 8, kClipShare = 4, kAdamShare = 2;  // units of a workgroup's share
 // Units of a launch, most.  The passes that write go over long lists in several launches: in one, the workgroups on
 // different parts of the chip drift apart, and reads and writes that far apart cost bandwidth.  AdamW of 1.5e9 weights
-// (with its norm), us: 8280 in one launch, 7990 in launches of 2^18 units, 7890 of 2^17, 7800 of 2^16, 7810 of 2^15; of
-// 41e6 weights 215, 212 in launches of 2^16, 221 of 2^15, 237 of 2^14.  The norm only reads: 2200 for 7.6e9 gradients
-// in one launch, 2470 in launches of 2^18.
+// (with its norm), us: 7840 in one launch, 7660 in launches of 2^18 units, 7580 of 2^17, 7580 of 2^16, 7630 of 2^15, 7790 of
+// 2^14; of 41e6 weights 201 in launches of 2^16 and more, 209 of 2^15, 223 of 2^14.  The norm only reads: 2200 for 7.6e9
+// gradients in one launch, 2470 in launches of 2^18.
 constexpr uint32_t kNormUnits = 1u << 30, kClipUnits = 1u << 18, kAdamUnits = 1u << 16;
 // Workgroups of a launch of the clip, which take several shares where there are more: usually there is nothing to clip,
 // and then they are what the launch costs.  7.6e9 bf16 gradients, us with nothing to clip and to clip them: 139 and 4870;

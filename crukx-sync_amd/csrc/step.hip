@@ -673,8 +673,8 @@ __device__ __forceinline__ void write_no_policy(const RowsIn &in, const PolicyOu
 // caches, and its gradient written.  A row of 152064 is 304 KB: with one workgroup of 1024 on each CU the rows in work
 // are 78 MB, of which 128 KB a row are in LDS; the 256 MB last-level cache keeps the rest from the first pass to the
 // second, so HBM sees one read and one write (with the first pass read past the caches 16384 rows of 152064 took 2517 us
-// instead of 1907).  Bound by the mix of reads and writes: those rows, a tenth of them masked (9.5 GB), take 1750 us,
-// 5.4 TB/s; when they took 1843, 1834 with multiplies for the exponentials and 1739 without the second read at all.
+// instead of 1907).  Bound by the mix of reads and writes: those rows, a tenth of them masked (9.5 GB), take this kernel
+// 1750 us, 5.4 TB/s; when it took 1843, 1834 with multiplies for the exponentials and 1739 without the second read at all.
 template <typename T, int BLOCK, uint32_t HOLD>
 __global__ __launch_bounds__(BLOCK) void k_policy(RowsIn in, PolicyIn p, PolicyOut o) {
     __shared__ Stat lds[BLOCK / 64];
@@ -874,8 +874,8 @@ __global__ __launch_bounds__(256) void k_clip(NormList l, const float *norm, flo
 
 // One element's step.  The weight is the new master rounded once more, so the master is rounded first.  The decay's
 // factor is held in 64 bits and joins the update before the one rounding: in 32 bits 1 - lr * weight_decay is 1 where the
-// product is under 3e-8 (a rate of 1e-6 with a decay of 0.01), and every master would miss its decay alike.  That costs
-// nothing next to the memory: 1.5e9 weights with their norm 7770-7790 us, 7750-7760 with the 32-bit factor.
+// product is under 3e-8 (a rate of 1e-6 with a decay of 0.01), and every master would miss its decay alike.  It costs
+// nothing next to the memory: 1.5e9 weights with their norm 7770-7790 us, and 7750-7760 with the 32-bit factor on that card.
 __device__ __forceinline__ void adam_one(const AdamArgs &a, float g, float &w, float &m, float &v) {
     m = a.beta1 * m + a.one_less_beta1 * g;
     v = a.beta2 * v + a.one_less_beta2 * (g * g);
@@ -954,9 +954,9 @@ __device__ __forceinline__ void adam_range(const AdamList &l, const AdamArgs &a,
     }
 }
 
-// Reads 14 bytes an element (bf16 gradients) and writes 14: 1.5e9 weights (43.2 GB) in 7.35 ms, 5.9 TB/s, over the rate
-// of a copy.  Small shares (2048 elements a workgroup, two rounds of its threads) keep every CU supplied to the end: with
-// the norm, and in launches of 72 tensors, 8.1 ms; 8.4 with shares of 8192, 8.8 of 32768.
+// Reads 14 bytes an element (bf16 gradients) and writes 14: 1.5e9 weights (43.2 GB) in 24 launches of together 6.84 ms,
+// 6.3 TB/s, over the rate of a copy.  Small shares (2048 elements a workgroup, two rounds of its threads) keep every CU
+// supplied to the end: with the norm 7.58 ms, 7.69 with shares of 4096, 7.80 of 8192, 8.29 of 32768.
 template <typename W, typename G>
 __global__ __launch_bounds__(256) void k_adamw(AdamList l, AdamArgs a) {
     const float f = a.norm ? clip_factor(*a.norm, a.max_norm) : 1.0f;
@@ -1000,7 +1000,8 @@ namespace {
 // workgroup's threads without a vector each; of long rows more workgroups hold more at once than the last-level cache
 // keeps for the loss's second pass.  Loss and gradient of 16000 rows of bf16, us with 64 / 256 / 1024 threads: 500 logits
 // 23 / 45 / 141, 4096: 56 / 63 / 153, 8192: 110 / 96 / 192, 32768: 459 / 390 / 411, 65536: 1034 / 835 / 749.  Scores: 500:
-// 9 / 21 / 78, 8192: 43 / 45 / 104, 65536: 314 / 302 / 308; 4000 rows of 152064: - / 182 / 175.
+// 9 / 21 / 78, 8192: 43 / 45 / 104, 65536: 314 / 302 / 308; 4000 rows of 152064: - / 182 / 175.  (At 256 to some 2000 rows,
+// where larger workgroups would fill the CUs better, the rule has not been measured.)
 constexpr uint64_t kWaveBytes = 8192, kScoreShort = 131072, kPolicyShort = 65536;
 
 template <typename T>
