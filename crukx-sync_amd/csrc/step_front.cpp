@@ -167,6 +167,8 @@ crx_logits logits_of(const Tensor &x, const Tensor &tokens, const Tensor &mask, 
     o.seqs = dim == 2 ? 1 : (uint64_t)x.size(0);
     o.tokens = (uint64_t)x.size(dim - 2);
     o.vocab = (uint64_t)x.size(dim - 1);
+    // (the library's own check comes after the results' allocation)
+    if (o.tokens && o.seqs > ((1ULL << 31) - 1) / o.tokens) bad("logits of 2^31 or more positions are not supported");
     o.stride_seq = dim == 2 ? 0 : x.stride(0);
     o.stride_token = x.stride(dim - 2);
     o.dtype = type;

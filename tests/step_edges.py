@@ -433,3 +433,13 @@ def adamw_of_every_pair_of_types_and_of_all_in_one_call(dev):
         crukx_sync.adamw_step(*s, step=5, lr=1e-3, weight_decay=0.1, grad_norm=norm, max_norm=1.0)
         for k in s[0]:
             _check_step(before, s, k, ref.factor(float(norm), 1.0))
+
+
+@edge
+def too_many_positions_are_refused_before_anything_is_allocated(dev):
+    """2^48 positions, as views without memory of their own; the results would take a petabyte."""
+    x, y, f = (t[:1].expand(1 << 24, 1 << 24, *t.shape[1:]) for t in _positions(dev))
+    for call in (lambda: crukx_sync.token_logprobs(x, y, entropy=True), lambda: crukx_sync.policy_loss(x, y, f, f),
+                 lambda: crukx_sync.policy_loss_grad(x, y, f, f), lambda: crukx_sync.token_logprobs(x.detach().requires_grad_(), y)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
